@@ -712,15 +712,21 @@ int dfa3d_embedding_grad_scale(const void *table, const void *index, int index_b
   return hip_result(dfa3d::launch_embedding_grad_scale(a, dtype, (hipStream_t)stream), fn);
 }
 
+static int check_embedding_table(const char *fn, int index_bytes, long long R, int N, int V, int H, int E, int dtype) {
+  if (int rc = check_embedding(fn, index_bytes, R, N, V, H, E, dtype)) return rc;
+  if (dfa3d::embedding_too_many(R, N)) return fail(DFA3D_ERANGE, "%s: at most 2^30 places of more than 2^20 batch elements in all (R=%lld N=%d)", fn, R, N);
+  return 0;
+}
+
 size_t dfa3d_embedding_grad_table_workspace_bytes(long long R, int N, int V, int H, int E, int dtype) {
-  if (check_embedding("dfa3d_embedding_grad_table_workspace_bytes", 8, R, N, V, H, E, dtype)) return 0;
+  if (check_embedding_table("dfa3d_embedding_grad_table_workspace_bytes", 8, R, N, V, H, E, dtype)) return 0;
   return dfa3d::embedding_workspace_bytes(R, N, V, H, E, dtype);
 }
 
 int dfa3d_embedding_grad_table(const void *table, const void *index, int index_bytes, const void *scale, const void *grad_out, void *grad_table,
                                void *grad_scale, void *workspace, size_t workspace_bytes, long long R, int N, int V, int H, int E, double mul, int dtype, void *stream) {
   const char *fn = "dfa3d_embedding_grad_table";
-  if (int rc = check_embedding(fn, index_bytes, R, N, V, H, E, dtype)) return rc;
+  if (int rc = check_embedding_table(fn, index_bytes, R, N, V, H, E, dtype)) return rc;
   REQUIRE_PTR(fn, index); REQUIRE_PTR(fn, grad_out); REQUIRE_PTR(fn, grad_table); REQUIRE_PTR(fn, workspace);
   if (grad_scale != nullptr) REQUIRE_PTR(fn, table);
   if (workspace_bytes < dfa3d::embedding_workspace_bytes(R, N, V, H, E, dtype) || ((uintptr_t)workspace & 255) != 0)

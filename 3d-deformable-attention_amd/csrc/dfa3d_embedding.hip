@@ -709,11 +709,20 @@ static int table_chunk(int N, int H, int E, int vec) {
 // at work while wavefronts add up one after the other many batch elements of each of an entry's places.  (Batch elements x places of entries x heads x elements in
 // float, gradients on the device: 1000 x 5 of 100 x 256 188 us of a pass and 47, 500 x 100 of 50 x 8 x 32 1912 and 62, 256 x 256 of 256 x 768 100 and 66, 64 x 250 of
 // 1000 x 256 31 and 26; 64 x 1000 of 1000 x 256 36 and 48, 32 x 300 of 300 x 8 x 256 37 and 44, 16 x 1000 of 1000 x 256 15 and 24.)
+// With more than 2^20 places in all, ordering them costs: there the pieces of an index of many places count as entries do.  (Likewise, gradients on the device, one
+// after the other and as places of their own: 20000 x 100 of 100 x 256 10191 us and 433, 2000 x 1000 of 1000 x 64 1075 and 212, 128 x 10000 of 100 x 256 481 and 292,
+// 16 x 100000 of 100 x 8 104 and 94; left one after the other 64 x 20000 of 100 x 256 290.)  And more than 2^20 batch elements always, as one float adds up those of
+// a place that are not places of their own.
+constexpr long long kMostPlaces = 1LL << 30, kSerialElements = 1LL << 20;
 static bool spread_over(long long R, int N, int V, int H, int E, int vec) {
+  if (R < 8 || R > kMostPlaces / N) return false;
   const int lanes = table_lanes(E, vec), slices = (E + lanes * vec - 1) / (lanes * vec), hb = heads_at_once(H), entries = std::min(N, V);
-  const long long waves = (long long)entries * slices * ((H + hb - 1) / hb) / (kWave / lanes);
-  return R >= 8 && R <= (1 << 20) / N && R * N / entries >= 128 && waves < 1024;
+  const int runs = R * N > (1 << 20) ? std::max(entries, N / table_chunk(N, H, E, vec)) : entries;
+  const long long waves = (long long)runs * slices * ((H + hb - 1) / hb) / (kWave / lanes);
+  return R > kSerialElements || (R * N / entries >= 128 && waves < 1024);
 }
+// Batch elements that would have to be places of their own, and are more than can be.
+bool embedding_too_many(long long R, int N) { return R > kSerialElements && R > kMostPlaces / N; }
 static size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 // What the ordering leaves and what it works in, from `ws` on (or nullptr: how large that is).
 struct OrderPlan {

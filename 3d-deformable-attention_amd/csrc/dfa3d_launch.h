@@ -217,6 +217,7 @@ hipError_t launch_embedding(const EmbeddingArgs &a, int dtype, hipStream_t strea
 hipError_t launch_embedding_grad_scale(const EmbeddingArgs &a, int dtype, hipStream_t stream);
 hipError_t launch_embedding_grad_table(const EmbeddingArgs &a, int dtype, hipStream_t stream);
 size_t embedding_workspace_bytes(long long R, int N, int V, int H, int E, int dtype);
+bool embedding_too_many(long long R, int N);      // for the table's gradient
 
 // Group norm with an activation (dfa3d_norm.hip): x, y, grad_y, grad_x (B, S, C), weight, bias and their gradients (C) or nullptr, level_start (L) or
 // nullptr (one level), stats (B, L, G, 2).

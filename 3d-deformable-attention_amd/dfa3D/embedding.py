@@ -108,7 +108,8 @@ def scaled_embedding(table, index, scale=None, plus=None, mul=1.0):
     ``mul``: a number.  Returns (..., *index.shape, E) of the table's type; sums are formed in float32 (float64).
 
     A place whose index is negative or not below V (the padding of a list) takes what ``plus`` holds there, and no gradient goes through it.
-    Gradients of the table are formed in an order that the sizes decide, without atomics: the same every time."""
+    Gradients of the table are formed in an order that the sizes decide, without atomics: the same every time.  They are refused where more than 2^20 batch
+    elements have more than 2^30 places in all."""
     mul = float(mul)
     if (here := native_for(table)) is not None and (got := here[0].embedding(here[1], here[2], table, index, scale, plus, mul)) is not None:
         return got

@@ -337,7 +337,7 @@ int dfa3d_dropout(const void *x, const void *residual, void *y, const int64_t *s
  *   grad_table: grad_table[v,h,:] = mul * sum over the n with index[n] = v and every r, in an order that the sizes decide, of scale[r,n,h] grad_out[r,n,:]; every
  *               element written, no atomics on the sums (the same result every time); grad_scale as well, in the same pass over the rows, unless it
  *               is NULL (table is not read then).  `workspace`: 256-byte aligned device memory of the size that the
- *               other function gives; its contents are irrelevant.
+ *               other function gives; its contents are irrelevant.  R N is at most 2^30 where R is more than 2^20.
  * The gradient of plus is grad_out.  dtype DFA3D_F32, DFA3D_F64, or DFA3D_BF16: table, plus, out and their gradients bfloat16, scale and its gradient
  * float, sums in float and rounded once. */
 int dfa3d_embedding(const void *table, const void *index, int index_bytes, const void *scale, const void *plus, void *out, long long R, int N, int V, int H,

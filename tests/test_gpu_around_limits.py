@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import test_gpu_norm as norm_checks
+from dfa3D.embedding import scaled_embedding
 
 pytestmark = pytest.mark.gpu
 
@@ -17,3 +18,52 @@ def test_norm_of_values_whose_squares_are_too_large(B, S, C, G, start, dtype):
     x = (2.0 ** 64 * 1.5 + step * torch.randint(-2, 3, (B, S, C), device="cuda")).to(dtype)
     assert bool(x.isfinite().all()) and bool((x.double() >= 2.0 ** 64).all())
     norm_checks.check(x, G, *norm_checks.params(C, dtype), start=start, act="silu")
+
+
+def whole_sums(R, N, V, H, E, dtype, scaled, index, seed=0):
+    """The gradients of a table and of its scales where every sum is one of whole numbers below 2^24, which float holds exactly whatever the order: what is lost or
+    counted twice shows, and only the last rounding to bfloat16 is left."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    whole = lambda low, high, *shape: torch.randint(low, high + 1, shape, generator=g, device="cuda")
+    lead = () if R is None else (R,)
+    table = whole(-3, 3, *((V, H, E) if H else (V, E))).to(dtype).requires_grad_()
+    wide = torch.float64 if dtype == torch.float64 else torch.float32
+    scale = whole(1, 2, *lead, N, *((H,) if H else ())).to(wide).requires_grad_() if scaled else None
+    plus = torch.zeros(*lead, N, E, dtype=dtype, device="cuda") if lead and not scaled else None
+    grad = whole(-2, 4, *lead, N, E).to(dtype)
+    out = scaled_embedding(table, index, scale=scale, plus=plus)
+    got = torch.autograd.grad(out, (table, scale) if scaled else table, grad)
+    there = (index >= 0) & (index < V)
+    at = index.long()[there]
+    rows = grad.reshape(-1, N, E)[:, there]
+    want = torch.zeros(V, max(H, 1), E, dtype=torch.int64, device="cuda")
+    by = None if scale is None else scale.detach().reshape(len(rows), N, max(H, 1))[:, there].long()
+    for r0 in range(0, len(rows), 64):
+        piece = rows[r0:r0 + 64].long()[:, :, None, :].expand(-1, -1, max(H, 1), -1)
+        want.index_add_(0, at, (piece if by is None else piece * by[r0:r0 + 64, :, :, None]).sum(0))
+    assert int(want.abs().max()) < 2 ** 24
+    assert torch.equal(got[0], want.view(table.shape).double().to(dtype))
+    if scaled:
+        dots = torch.zeros(len(grad.reshape(-1, N, E)), N, max(H, 1), dtype=torch.int64, device="cuda")
+        dots[:, there] = (rows.long()[:, :, None, :] * table.detach().reshape(V, max(H, 1), E)[at].long()[None]).sum(-1)
+        assert torch.equal(got[1], dots.view(scale.shape).to(wide))
+
+
+@pytest.mark.parametrize("dtype,scaled", [(torch.float32, True), (torch.bfloat16, False)])
+@pytest.mark.parametrize("R,N,V,H,E", [(10000, 100, 100, 0, 64), (20000, 100, 100, 0, 64), (20000, 60, 100, 2, 12), (3000, 700, 131073, 0, 8), (64, 20000, 100, 0, 256), (9, 120000, 50, 3, 16)])
+def test_lookup_of_many_batch_elements(R, N, V, H, E, dtype, scaled):
+    """On both sides of 2^20 places of all batch elements, and of the rule by which those are places of their own."""
+    index = torch.randint(-1, V + 1, (N,), generator=torch.Generator().manual_seed(R)).cuda()
+    index[N // 2] = V - 1
+    whole_sums(R, N, V, H, E, dtype, scaled, index)
+
+
+def test_lookup_of_more_batch_elements_than_float_counts():
+    """One place of 2^25 batch elements whose gradients are ones: a float that adds them up one after the other stops at 2^24."""
+    R = 2 ** 25
+    for scaled in (False, True):
+        table = torch.randn(3, 4, device="cuda", requires_grad=True)
+        ones = torch.ones(R, 1, device="cuda") if scaled else None
+        out = scaled_embedding(table, torch.tensor([1], device="cuda"), scale=ones, plus=None if scaled else torch.zeros(R, 1, 4, device="cuda"))
+        grad, = torch.autograd.grad(out, table, torch.ones_like(out))
+        assert torch.equal(grad, torch.tensor([0.0, R, 0.0], device="cuda")[:, None].expand(3, 4))
