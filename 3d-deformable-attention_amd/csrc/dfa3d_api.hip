@@ -747,6 +747,7 @@ static int check_norm(const char *fn, int B, int S, int C, int G, int L, int act
   if (act != DFA3D_ACT_NONE && act != DFA3D_ACT_RELU && act != DFA3D_ACT_SILU) return fail(DFA3D_EINVAL, "%s: unknown activation %d", fn, act);
   if (S > (1 << 30) || C > (1 << 20) || (long long)B * S > (1LL << 31))
     return fail(DFA3D_ERANGE, "%s: at most 2^30 keys, 2^31 in all, of 2^20 channels (B=%d S=%d C=%d)", fn, B, S, C);
+  if ((long long)B * L > (1 << 30)) return fail(DFA3D_ERANGE, "%s: at most 2^30 levels in all (B=%d L=%d)", fn, B, L);
   return 0;
 }
 static dfa3d::NormArgs norm_dims(int B, int S, int C, int G, int L, int act) {

@@ -36,6 +36,7 @@ struct NormDims {
   int cols, at_once;                   // threads of a key's pieces in a workgroup, and keys at once
   float per_col;                       // 1 / cols
   int tile, tiles, slots;              // keys of a tile, tiles and slots of a batch element
+  unsigned first;                      // tile of the first batch element and on that the launch begins with
   float per_piece;                     // 1 / group
   int group, abreast, cells, blocks;   // pieces of a group and groups side by side; the statistics' parts of a tile: one per group, or per block of a group's pieces where those are more than a workgroup
 };
@@ -110,8 +111,9 @@ __global__ __launch_bounds__(kNormBlock) void norm_parts_kernel(const T *__restr
     pieces = min(d.group - block * d.cols, d.cols);
   }
   const bool on = row < d.at_once && piece < d.C / VEC && (d.blocks == 1 || col < pieces);
-  const long long b = blockIdx.x / d.tiles;
-  const int tile = blockIdx.x - (int)b * d.tiles, k0 = tile * d.tile, k1 = min(k0 + d.tile, d.S);
+  const unsigned block = d.first + blockIdx.x;
+  const long long b = block / d.tiles;
+  const int tile = (int)(block - (unsigned)b * d.tiles), k0 = tile * d.tile, k1 = min(k0 + d.tile, d.S);
   const T *from = x + (b * d.S) * d.C + (long long)piece * VEC;
   A v[KEYS][VEC];
 #pragma unroll
@@ -305,9 +307,9 @@ __global__ __launch_bounds__(kNormBlock) void norm_apply_kernel(const T *__restr
   const int per = d.C / VEC, row = part_of(threadIdx.x, d.per_col), piece = blockIdx.y * d.cols + threadIdx.x - row * d.cols;
   const bool on = row < d.at_once && piece < per;
   // the tiles that were read last first: what of them is still in the caches need not come from memory again
-  const int block = gridDim.x - 1 - blockIdx.x;
+  const unsigned block = d.first + gridDim.x - 1 - blockIdx.x;
   const long long b = block / d.tiles;
-  const int tile = block - (int)b * d.tiles, k0 = tile * d.tile, k1 = min(k0 + d.tile, d.S);
+  const int tile = (int)(block - (unsigned)b * d.tiles), k0 = tile * d.tile, k1 = min(k0 + d.tile, d.S);
   const long long at = (b * d.S) * d.C + (long long)piece * VEC;
   // kAhead keys at once, the next ones on their way while these are worked on (the first ones while the levels are sorted)
   Raw<T, VEC> xs[2][kAhead], gs[2][BACK ? kAhead : 1];
@@ -382,8 +384,9 @@ __global__ __launch_bounds__(kNormBlock) void norm_grad_parts_kernel(const T *__
   sort_levels(level_start, d.L, d.S, s_first);
   const int per = d.C / VEC, row = part_of(threadIdx.x, d.per_col), piece = blockIdx.y * d.cols + threadIdx.x - row * d.cols;
   const bool on = row < d.at_once && piece < per;
-  const long long b = blockIdx.x / d.tiles;
-  const int tile = blockIdx.x - (int)b * d.tiles, k0 = tile * d.tile, k1 = min(k0 + d.tile, d.S);
+  const unsigned block = d.first + blockIdx.x;
+  const long long b = block / d.tiles;
+  const int tile = (int)(block - (unsigned)b * d.tiles), k0 = tile * d.tile, k1 = min(k0 + d.tile, d.S);
   const int g = on ? piece * VEC / (d.C / d.G) : 0;
   A w[VEC], bb[VEC];
   channel_params<VEC>(weight, bias, on ? piece * VEC : 0, w, bb);
@@ -760,12 +763,20 @@ static NormDims parts_dims(const NormArgs &a, int vec) {
   d.slots = d.tiles + a.L - 1;
   return d;
 }
-static dim3 parts_grid(const NormDims &d) { return dim3((unsigned)((long long)d.B * d.tiles), (d.cells + d.abreast - 1) / d.abreast); }
-static dim3 norm_grid(const NormDims &d, int vec) { return dim3((unsigned)((long long)d.B * d.tiles), (d.C / vec + d.cols - 1) / d.cols); }
-
 static unsigned most_blocks(long long blocks) { return (unsigned)std::min(blocks, 1LL << 20); }
-// (a grid holds fewer than 2^32 threads)
-static bool grid_fits(const NormDims &d) { return (long long)d.B * d.tiles < (1LL << 32) / kNormBlock; }
+// launch(d, grid) for all tiles of all batch elements, `columns` workgroups each: in turns, as a grid holds fewer than 2^32 threads.
+constexpr long long kTurn = 1 << 23;
+template <typename F> static hipError_t in_turns(NormDims d, int columns, F launch) {
+  const long long all = (long long)d.B * d.tiles;
+  for (long long first = 0; first < all; first += kTurn) {
+    d.first = (unsigned)first;
+    launch(d, dim3((unsigned)std::min(kTurn, all - first), columns));
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
+}
+static int parts_columns(const NormDims &d) { return (d.cells + d.abreast - 1) / d.abreast; }
+static int norm_columns(const NormDims &d, int vec) { return (d.C / vec + d.cols - 1) / d.cols; }
 
 constexpr int kSerialParts = 8;
 // Ranges in which the gradients' parts are added up first, for few groups of many of them; 0: not.  (One after the other, and in
@@ -835,10 +846,10 @@ static hipError_t norm_forward(const NormArgs &a, hipStream_t stream) {
                                                                        : launch(norm_small_kernel<T, VEC, ACT, kSmallBlock>, kSmallBlock);
   }
   const NormDims k = norm_dims(a, VEC, apply_keys(a, VEC, (int)sizeof(T)));
-  if (!grid_fits(d) || !grid_fits(k)) return hipErrorInvalidConfiguration;
-  const dim3 grid = parts_grid(d);
-  hipLaunchKernelGGL((norm_parts_kernel<T, VEC, norm_keys(VEC)>), grid, dim3(kNormBlock), 0, stream, (const T *)a.x, a.level_start, (A *)a.workspace, d);
-  if (hipError_t e = hipGetLastError()) return e;
+  auto parts = [&](const NormDims &d, dim3 grid) {
+    hipLaunchKernelGGL((norm_parts_kernel<T, VEC, norm_keys(VEC)>), grid, dim3(kNormBlock), 0, stream, (const T *)a.x, a.level_start, (A *)a.workspace, d);
+  };
+  if (hipError_t e = in_turns(d, parts_columns(d), parts)) return e;
   const long long units = (long long)d.B * d.L * d.G;
   const int lanes = unit_lanes(units, (long long)d.tiles * d.blocks, kHeldParts);
   auto stats = [&](auto kernel) {
@@ -848,15 +859,15 @@ static hipError_t norm_forward(const NormArgs &a, hipStream_t stream) {
   };
   if (hipError_t e = lanes == 4 ? stats(norm_stats_kernel<A, 4>) : lanes == 16 ? stats(norm_stats_kernel<A, 16>) : lanes == 64 ? stats(norm_stats_kernel<A, 64>)
                                                                                                         : stats(norm_stats_kernel<A, kNormBlock>)) return e;
-  hipLaunchKernelGGL((norm_apply_kernel<T, VEC, ACT, false>), norm_grid(k, VEC), dim3(kNormBlock), 0, stream, (const T *)a.x, (const T *)nullptr, (const A *)a.weight, (const A *)a.bias,
-                     a.level_start, (const A *)a.stats, (const A *)nullptr, (T *)a.y, k, ParamGrads{});
-  return hipGetLastError();
+  return in_turns(k, norm_columns(k, VEC), [&](const NormDims &k, dim3 grid) {
+    hipLaunchKernelGGL((norm_apply_kernel<T, VEC, ACT, false>), grid, dim3(kNormBlock), 0, stream, (const T *)a.x, (const T *)nullptr, (const A *)a.weight, (const A *)a.bias,
+                       a.level_start, (const A *)a.stats, (const A *)nullptr, (T *)a.y, k, ParamGrads{});
+  });
 }
 template <typename T, int VEC, int ACT>
 static hipError_t norm_backward(const NormArgs &a, hipStream_t stream) {
   typedef typename Sum<T>::type A;
   const NormDims d = norm_dims(a, VEC, grad_keys(a, VEC)), k = norm_dims(a, VEC, apply_keys(a, VEC, (int)sizeof(T)));
-  if (!grid_fits(k) || !grid_fits(d)) return hipErrorInvalidConfiguration;
   A *parts = (A *)a.workspace;
   double *channels = (double *)((char *)a.workspace + grad_parts_bytes(a, VEC, sizeof(A)));
   A *sums = (A *)((char *)channels + rounded((size_t)a.B * a.L * a.C * 2 * sizeof(double)));
@@ -869,9 +880,11 @@ static hipError_t norm_backward(const NormArgs &a, hipStream_t stream) {
                        one ? (A *)a.grad_bias : nullptr, (T *)a.grad_x, d);
     if (one) return hipGetLastError();
   } else {
-    hipLaunchKernelGGL((norm_grad_parts_kernel<T, VEC, ACT>), norm_grid(d, VEC), dim3(kNormBlock), 0, stream, (const T *)a.x, (const T *)a.grad_y, (const A *)a.weight,
-                       (const A *)a.bias, a.level_start, (const A *)a.stats, parts, d);
-    if (hipError_t e = hipGetLastError()) return e;
+    auto grad_parts = [&](const NormDims &d, dim3 grid) {
+      hipLaunchKernelGGL((norm_grad_parts_kernel<T, VEC, ACT>), grid, dim3(kNormBlock), 0, stream, (const T *)a.x, (const T *)a.grad_y, (const A *)a.weight, (const A *)a.bias,
+                         a.level_start, (const A *)a.stats, parts, d);
+    };
+    if (hipError_t e = in_turns(d, norm_columns(d, VEC), grad_parts)) return e;
     const int K = fold_ranges(d);
     if (K > 0) {
       hipLaunchKernelGGL((norm_fold_kernel<A>), dim3((unsigned)(d.B * d.L * K), (d.C * 2 + kNormBlock - 1) / kNormBlock), dim3(kNormBlock), 0, stream, parts, a.level_start,
@@ -913,11 +926,12 @@ static hipError_t norm_backward(const NormArgs &a, hipStream_t stream) {
     return hipGetLastError();
   }
   if (small || a.grad_x == nullptr) return hipSuccess;
-  dim3 grid = norm_grid(k, VEC);
-  grid.x += params.blocks;
-  hipLaunchKernelGGL((norm_apply_kernel<T, VEC, ACT, true>), grid, dim3(kNormBlock), 0, stream, (const T *)a.x, (const T *)a.grad_y, (const A *)a.weight, (const A *)a.bias,
-                     a.level_start, (const A *)a.stats, sums, (T *)a.grad_x, k, params);
-  return hipGetLastError();
+  return in_turns(k, norm_columns(k, VEC), [&](const NormDims &k, dim3 grid) {
+    grid.x += params.blocks;
+    hipLaunchKernelGGL((norm_apply_kernel<T, VEC, ACT, true>), grid, dim3(kNormBlock), 0, stream, (const T *)a.x, (const T *)a.grad_y, (const A *)a.weight, (const A *)a.bias,
+                       a.level_start, (const A *)a.stats, sums, (T *)a.grad_x, k, params);
+    params.blocks = 0;                                       // (formed)
+  });
 }
 
 template <typename T, int VEC>

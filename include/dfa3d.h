@@ -353,7 +353,8 @@ int dfa3d_embedding_grad_table(const void *table, const void *index, int index_b
  *   y = act((x - mean) / sqrt(variance + eps) * weight + bias),  variance about the mean, divided by the count
  * level_start (L) int64: a level begins there and ends where the next one begins, the last one at S; in any order, and NULL with L = 1 for one level of all
  * keys.  Keys before the first level come out as zeros, as do their gradients.  weight (C) or NULL (ones), bias (C) or NULL (zeros).  stats (B, L, groups, 2):
- * means and 1 / sqrt(variance + eps), levels in the order of their keys; written by the one, read by the other.
+ * means and 1 / sqrt(variance + eps), levels in the order of their keys; written by the one, read by the other.  At most 2^30 keys of 2^20 channels in 16 levels, and of
+ * all batch elements 2^31 keys and 2^30 levels.
  * dfa3d_group_norm_grad: grad_x (B, S, C), grad_weight and grad_bias (C) from grad_y, each not formed where it is NULL; no atomics (the same result every time).
  * `workspace`: 256-byte aligned device memory of the size that the other function gives (backward: 0 or 1); its contents are irrelevant.
  * dtype DFA3D_F32, DFA3D_F64, or DFA3D_BF16: x, y, grad_y and grad_x bfloat16, the others float, sums in float or double and results rounded once. */

@@ -23,3 +23,13 @@ def test_batch_elements_are_places_of_their_own():
         assert need(R, N, V, H, E, 0) == need(1, R * N, V, H, E, 0)
     for R, N, V, H, E in ((7, 200000, 1, 1, 256), (64, 2 ** 20, 100, 1, 256), (64, 2000, 2000, 8, 256)):
         assert need(R, N, V, H, E, 0) == need(1, N, V, H, E, 0)
+
+
+def test_a_norm_of_too_many_levels():
+    """Of all batch elements together, whose channels' sums are numbered in 31 bits."""
+    from dfa3D import _lib
+    lib = _lib.lib()
+    size = lib.dfa3d_group_norm_workspace_bytes
+    assert size(2 ** 26 + 1, 1, 8, 2, 16, 1, 0) == 0 and b"2^30 levels" in lib.dfa3d_last_error()
+    assert size(2 ** 30, 1, 8, 2, 1, 0, 0) > 0
+    assert lib.dfa3d_group_norm(ONE, NULL, NULL, ONE, ONE, ONE, ONE, 1 << 50, 2 ** 26 + 1, 1, 8, 2, 16, 1e-5, 0, 0, NULL) == -2

@@ -67,3 +67,13 @@ def test_lookup_of_more_batch_elements_than_float_counts():
         out = scaled_embedding(table, torch.tensor([1], device="cuda"), scale=ones, plus=None if scaled else torch.zeros(R, 1, 4, device="cuda"))
         grad, = torch.autograd.grad(out, table, torch.ones_like(out))
         assert torch.equal(grad, torch.tensor([0.0, R, 0.0], device="cuda")[:, None].expand(3, 4))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,S,start", [(17000000, 1, None), (2 ** 24 - 1, 1, None), (8400001, 2, (0, 1))])
+def test_norm_of_more_batch_elements_than_a_grid_holds(B, S, start, dtype):
+    """Tiles of all batch elements in turns."""
+    torch.manual_seed(S)
+    x = torch.empty(B, S, 8, device="cuda", dtype=dtype).normal_()
+    norm_checks.check(x, 2, *norm_checks.params(8, dtype), start=start)
+    torch.cuda.empty_cache()
