@@ -84,15 +84,13 @@ template <int ACT, typename A> __device__ __forceinline__ A through_activation(A
   return d;
 }
 
-// Two samples' count, mean and sum of squares about the mean as one's (T. Chan, G. Golub, R. LeVeque, 1979).  Where one is empty it is the other: its mean of zero says
-// nothing, and the other one's may have a square that is infinite, which times no elements is not a number.
+// Two samples' count, mean and sum of squares about the mean as one's (T. Chan, G. Golub, R. LeVeque, 1979).  Where one is empty (its mean is zero) it is the other: the square
+// of the other one's mean may be infinite, which times no elements is not a number.
 template <typename A> struct Moments { A n, mean, m2; };
 template <typename A> __device__ __forceinline__ Moments<A> joined(const Moments<A> &a, const Moments<A> &b) {
-  if (a.n == 0) return b;
   if (b.n == 0) return a;
-  const A n = a.n + b.n;
-  const A d = b.mean - a.mean, part = b.n / n;
-  return Moments<A>{n, a.mean + d * part, a.m2 + b.m2 + d * d * a.n * part};
+  const A n = a.n + b.n, d = b.mean - a.mean, part = b.n / n;
+  return Moments<A>{n, a.mean + d * part, a.m2 + b.m2 + (a.n != 0 ? d * d * a.n * part : (A)0)};
 }
 
 // parts (B, slots, cells): mean and sum of squares about it of a part's keys and a group's channels (or a block's of them)
