@@ -29,6 +29,7 @@
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <unordered_set>
 #include <utility>
 #include <vector>
 
@@ -806,22 +807,60 @@ void require_taken(const Outcome &o) {
 }
 Tensor bytes_like(const Tensor &t, size_t n) { return at::empty({(int64_t)n}, t.options().dtype(at::kByte)); }
 
-// Whether a graph that was made on the default stream holds the leaf: its node that takes the leaf's gradients is alive, and belongs to that stream.
-bool held_by_default_stream(const Tensor &leaf) {
-  if (!leaf.is_leaf()) return false;
-  const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
-  if (node == nullptr) return false;
-  const auto stream = node->stream();
-  return stream.has_value() && stream->id() == c10::hip::getDefaultHIPStream(leaf.get_device()).id();      // (its device is of type cuda, the other's hip)
+// Whether a backward from here on comes to a node of the default stream: one that was made there, or a leaf's that takes its gradients and is alive because a graph that
+// was made there is.  (A node's stream is of type cuda, the other one of type hip: their numbers are compared.)
+bool of_default_stream(torch::autograd::Node &node) {
+  const auto stream = node.stream();
+  return stream.has_value() && stream->id() == c10::hip::getDefaultHIPStream(stream->device_index()).id();
+}
+bool leads_to_default_stream(const Tensor &t) {
+  if (!t.requires_grad()) return false;
+  if (t.is_leaf()) {
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    return node != nullptr && of_default_stream(*node);
+  }
+  std::vector<torch::autograd::Node *> left{t.grad_fn().get()};      // (which the tensor keeps alive, and they the next ones)
+  std::unordered_set<torch::autograd::Node *> seen(left.begin(), left.end());
+  while (!left.empty()) {
+    torch::autograd::Node *node = left.back();
+    left.pop_back();
+    if (of_default_stream(*node)) return true;
+    for (const auto &edge : node->next_edges())
+      if (edge.is_valid() && seen.insert(edge.function.get()).second) left.push_back(edge.function.get());
+  }
+  return false;
 }
 bool capturing(int64_t device) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   return hipStreamIsCapturing(c10::hip::getCurrentHIPStream(device).stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
 }
-// held(leaf) -> held_by_default_stream
+// held(tensor) -> leads_to_default_stream
 PyObject *held(PyObject *, PyObject *o) {
   HANDLE_TH_ERRORS
-  return PyBool_FromLong(THPVariable_Check(o) && THPVariable_Unpack(o).is_cuda() && held_by_default_stream(THPVariable_Unpack(o)));
+  return PyBool_FromLong(THPVariable_Check(o) && THPVariable_Unpack(o).is_cuda() && leads_to_default_stream(THPVariable_Unpack(o)));
+  END_HANDLE_TH_ERRORS
+}
+// The engine joins the default stream in a backward that comes to a node of it; a capture does not survive that, nor does the process.  So under a capture the call that
+// leads there is refused: false, with an error set.
+bool capture_survives(int64_t device, std::initializer_list<const Tensor *> operands) {
+  if (!c10::GradMode::is_enabled() || !capturing(device)) return true;
+  for (const Tensor *t : operands)
+    if (t->defined() && leads_to_default_stream(*t)) {
+      PyErr_SetString(PyExc_RuntimeError, "this call is captured and recorded for a backward while a graph of the same leaf that was made on the default stream is alive, "
+                                          "which ends the process in that backward: delete that graph's outputs before the capture, or capture the call under no_grad");
+      return false;
+    }
+  return true;
+}
+// refuse_capture(tensor or None, ...): the same for calls that are made step by step
+PyObject *refuse_capture(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  for (Py_ssize_t i = 0; i < nargs; ++i)
+    if (THPVariable_Check(args[i])) {
+      const Tensor &t = THPVariable_Unpack(args[i]);
+      if (t.is_cuda() && !capture_survives(t.get_device(), {&t})) return nullptr;
+    }
+  Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
 
@@ -929,13 +968,7 @@ template <typename F, typename Saved>
 PyObject *recorded_output(const Tensor &out, const Numbers &n, const Tensor &a, const Tensor &b, const Tensor &c, Saved saved) {
   const auto records = [](const Tensor &t) { return t.defined() && t.requires_grad(); };
   if (!c10::GradMode::is_enabled() || !(records(a) || records(b) || records(c))) return THPVariable_Wrap(out);
-  // The engine joins the default stream in the backward of what is recorded here, if a graph from there holds a leaf; a capture does not survive that, nor does the
-  // process.  So the call that leads there is refused.
-  if (capturing(out.get_device()) && ((records(a) && held_by_default_stream(a)) || (records(b) && held_by_default_stream(b)) || (records(c) && held_by_default_stream(c)))) {
-    PyErr_SetString(PyExc_RuntimeError, "this call is captured and recorded for a backward while a graph of the same leaf that was made on the default stream is alive, "
-                                        "which ends the process in that backward: delete that graph's outputs before the capture");
-    return nullptr;
-  }
+  if (!capture_survives(out.get_device(), {&a, &b, &c})) return nullptr;
   const auto there = [](const Tensor &t) { return t.defined() ? MayBe(t) : MayBe(); };
   const variable_list kept = saved(records(a), records(b), records(c));
   return THPVariable_Wrap(F::apply((const Tensor *)&out, (const variable_list *)&kept, (const Numbers *)&n, there(a), there(b), there(c)));
@@ -1118,6 +1151,7 @@ PyMethodDef methods[] = {
     {"embedding", as_method(embedding), METH_FASTCALL, nullptr},
     {"group_norm", as_method(group_norm), METH_FASTCALL, nullptr},
     {"held", held, METH_O, nullptr},
+    {"refuse_capture", as_method(refuse_capture), METH_FASTCALL, nullptr},
     {"set_python_backward_around", set_python_backward_around, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -4,7 +4,7 @@ import torch
 
 from . import _lib
 from ._operands import as_read, check_beside
-from .recording import Noted, OperatorFunction, native_for
+from .recording import Noted, OperatorFunction, native_for, refuse_capture
 
 __all__ = ["dropout", "DropoutFunction"]
 
@@ -80,4 +80,5 @@ def dropout(x, p, seed, site=0, residual=None):
     site = int(site)
     if not 0 <= site < 2 ** 63:
         raise ValueError(f"site must be a non-negative int of 63 bits, got {site}")
+    refuse_capture(x, residual)
     return DropoutFunction.apply(x, residual, p, seed, site)

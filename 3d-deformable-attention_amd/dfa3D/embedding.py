@@ -7,7 +7,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._operands import as_read, check_beside
-from .recording import Noted, OperatorFunction, native_for
+from .recording import Noted, OperatorFunction, native_for, refuse_capture
 
 __all__ = ["scaled_embedding", "ScaledEmbeddingFunction"]
 
@@ -131,4 +131,5 @@ def scaled_embedding(table, index, scale=None, plus=None, mul=1.0):
         if lead is None:
             lead = tuple(t.shape[:max(t.dim() - len(tail), 0)])
         check_beside(table, t, name, (*lead, *tail), dtype)
+    refuse_capture(table, scale, plus)
     return ScaledEmbeddingFunction.apply(table, index, scale, plus, mul)

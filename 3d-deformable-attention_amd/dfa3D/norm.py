@@ -5,7 +5,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._operands import as_read, check_beside
-from .recording import Noted, OperatorFunction, native_for
+from .recording import Noted, OperatorFunction, native_for, refuse_capture
 
 __all__ = ["level_group_norm", "LevelGroupNormFunction"]
 
@@ -119,4 +119,5 @@ def level_group_norm(x, num_groups, weight=None, bias=None, level_start_index=No
         check_beside(x, level_start_index, "level_start_index", level_start_index.shape, torch.int64)
         if level_start_index.dim() != 1 or not 0 < len(level_start_index) <= _lib.MAX_LEVELS:
             raise RuntimeError(f"level_start_index must hold 1 to {_lib.MAX_LEVELS} levels, got {tuple(level_start_index.shape)}")
+    refuse_capture(x, *params)
     return LevelGroupNormFunction.apply(x, *params, level_start_index, num_groups, eps, _lib.ACTIVATIONS[act])

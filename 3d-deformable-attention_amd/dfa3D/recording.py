@@ -5,7 +5,7 @@ from torch.autograd.function import Function
 
 from . import _ext, _lib
 
-__all__ = ["OperatorFunction", "native_for", "Noted", "SCORE", "STAGE2", "PLAIN", "FUSED", "WEIGHT_UPDATE"]
+__all__ = ["OperatorFunction", "native_for", "Noted", "refuse_capture", "SCORE", "STAGE2", "PLAIN", "FUSED", "WEIGHT_UPDATE"]
 
 SCORE, STAGE2, PLAIN, FUSED, WEIGHT_UPDATE = range(5)        # what the binding module calls and records as a whole
 
@@ -43,6 +43,13 @@ def native_for(t):
         return None
     at = torch._C._cuda_getDevice()
     return native, at, torch._C._cuda_getCurrentRawStream(at)
+
+
+def refuse_capture(*operands):
+    """Before a call is recorded step by step under a capture: refuses it where the binding module refuses those that it records itself, where a backward would come to
+    what was recorded on the default stream.  Without that module there is nobody to ask."""
+    if not torch.compiler.is_compiling() and (native := _lib.binding()) is not None:
+        native.refuse_capture(*operands)
 
 
 class OperatorFunction(Function):
