@@ -77,3 +77,35 @@ def test_norm_of_more_batch_elements_than_a_grid_holds(B, S, start, dtype):
     x = torch.empty(B, S, 8, device="cuda", dtype=dtype).normal_()
     norm_checks.check(x, 2, *norm_checks.params(8, dtype), start=start)
     torch.cuda.empty_cache()
+
+
+def _one_entry(N, V):
+    index = torch.randint(0, V, (N,))
+    index[N // 3:N // 2], index[N // 2:N // 2 + 40] = V - 1, V // 2
+    outside = torch.rand(N) < 0.2
+    index[outside] = torch.tensor([-1, V, -V - 5, 2 ** 31 - 1])[torch.randint(0, 4, (int(outside.sum()),))]
+    return index
+
+
+def _low_entries(N, V):
+    return ((torch.rand(N, dtype=torch.float64) * 11.0).exp() - 1).long().clamp(max=V - 1)
+
+
+def _long_runs(N, V):
+    index = torch.randint(0, V, (N,))
+    index[N // 4:N // 2], index[N // 2:N // 2 + 17], index[-700:] = V - 1, 7, min(V - 1, 262144)
+    return index
+
+
+@pytest.mark.parametrize("index_type", [torch.int32, torch.int64])
+@pytest.mark.parametrize("made,N,V", [(_one_entry, 65536, 131072), (_one_entry, 65537, 1), (_one_entry, 70001, 1024), (_one_entry, 100003, 2 ** 20 + 1), (_one_entry, 131071, 3),
+                                      (_one_entry, 70000, 2 ** 22 + 2047), (_low_entries, 60000, 90000), (_low_entries, 90000, 60000), (_long_runs, 20011, 400001), (_long_runs, 30000, 50),
+                                      (_long_runs, 1048576, 500), (_low_entries, 1048577, 50000)])
+def test_lookup_sums_of_whole_numbers(made, N, V, index_type):
+    """Entries of very many places, whose sums are cut in pieces, in both ways of ordering: no place is lost or counted twice."""
+    torch.manual_seed(N + V)
+    index = made(N, V).to(index_type).cuda()
+    whole_sums(None, N, V, 0, 6, torch.float32, True, index)
+    whole_sums(2, N, V, 2, 4, torch.float32, True, index)
+    whole_sums(None, N, V, 5, 8, torch.bfloat16, True, index)
+    whole_sums(None, N, V, 0, 40, torch.bfloat16, False, index)
