@@ -3,7 +3,9 @@ import pytest
 import torch
 
 import test_gpu_norm as norm_checks
+from dfa3D.dropout import dropout
 from dfa3D.embedding import scaled_embedding
+from dfa3D.norm import level_group_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +111,31 @@ def test_lookup_sums_of_whole_numbers(made, N, V, index_type):
     whole_sums(2, N, V, 2, 4, torch.float32, True, index)
     whole_sums(None, N, V, 5, 8, torch.bfloat16, True, index)
     whole_sums(None, N, V, 0, 40, torch.bfloat16, False, index)
+
+
+@pytest.mark.parametrize("act", [None, "silu"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("S,C", [(127, 513), (64, 1023), (90, 721)])
+def test_norm_of_the_longest_sums_in_a_thread(S, C, dtype, act):
+    """One launch, one key at a time beside 513 to 1024 pieces of one channel: a thread adds up as many terms of a channel as there are keys, up to 127 (2^16 elements of
+    a group in 513 pieces), before anything is in double.  Bounds as in the tests of the norm, whose 80 u for sums are 136 u here: at most 1.7 times them."""
+    torch.manual_seed(S)
+    x = (torch.randn(1, S, C, device="cuda") + torch.randn(C, device="cuda")).to(dtype).requires_grad_()
+    w, b = (t.requires_grad_() for t in norm_checks.params(C, dtype))
+    y = level_group_norm(x, 1, w, b, act=act)
+    g = torch.randint(-4, 5, y.shape, device="cuda").to(dtype)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+    with torch.no_grad():
+        want = norm_checks.formulas(x, 1, w, b, None, 1e-5, act, g, dtype)
+    for got, (value, off), kind, name in ((y, want[0], dtype, "y"), (dx, want[1], dtype, "dx"), (dw, want[2], torch.float32, "dw"), (db, want[3], torch.float32, "db")):
+        norm_checks.close(got, value, 1.7 * off, kind, name)
+    if act is None:
+        assert torch.equal(db, g.double().sum((0, 1)).float())   # whole numbers: exact
+
+
+def test_dropout_draws_the_published_words():
+    """Philox4x32 of seven rounds at a counter and a key of zero, from the authors' table of known answers: an element is kept where p 2^32 is its word, and dropped where it
+    is one more."""
+    x = torch.ones(4, device="cuda")
+    for k, word in enumerate((0x5F6FB709, 0x0D893F64, 0x4F121F81, 0x4F730A48)):
+        assert dropout(x, word / 2.0 ** 32, 0, 0)[k] > 0 and dropout(x, (word + 1) / 2.0 ** 32, 0, 0)[k] == 0
