@@ -146,7 +146,7 @@ constexpr int kOrderWaves = 16, kOrderBlock = kOrderWaves * kWave;
 constexpr int kOrderGroups = 256, kXcds = 8;
 constexpr int kOrderPer = 512;         // (32 KB of counts)
 constexpr int kOrderAhead = 8;         // places of a lane asked for at once
-constexpr int kOrderLds = 60 << 10;    // for the counts, and for the places that the wavefronts keep from their first reading for the second: 256 to 640 each
+constexpr int kOrderLds = 60 << 10;    // for the counts, and for the places that the wavefronts keep from their first reading for the second: 256 to 576 each
 
 // A place as it stands in the index, in 32 bits: what lies outside the table comes out as no entry of it and not before any.
 template <bool SPREAD, typename I> __device__ __forceinline__ uint32_t raw_entry(const I *__restrict__ index, long long n, int period) {

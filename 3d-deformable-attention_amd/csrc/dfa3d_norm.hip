@@ -65,7 +65,8 @@ __device__ __forceinline__ void sort_levels(const int64_t *__restrict__ level_st
   __syncthreads();
 }
 
-// 1 / (1 + exp(-u)).  In float by the hardware's power of two and reciprocal: the rounding of u log2(e) weighs no more than that of u itself.  (The
+// 1 / (1 + exp(-u)).  In float by the hardware's power of two and reciprocal: the rounding of u log2(e) weighs no more than that of u itself, which has been computed (both
+// |u| 2^-24 of the gate, 5e-6 at u = -80); below u = -87 the gate is less than the least float that is not subnormal, and zero.  (The
 // library's exponential and a correct division: 6 x 30825 x 256 in bfloat16 61 us for 41.)
 __device__ __forceinline__ float gate_of(float u) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * -1.44269504088896341f)); }
 __device__ __forceinline__ double gate_of(double u) { return 1.0 / (1.0 + exp(-u)); }
@@ -206,7 +207,7 @@ static int unit_lanes(long long units, long long each, int held) {
 // it is little, and the counts of a large map leave float's whole numbers.
 // The parts of a group are few bytes of each line: what bounds this is that they come.  (6 x 30825 x 256 in float, four levels, neighbouring
 // groups anywhere and parts asked for in turn 12.3 us, groups side by side 9.6, parts asked for at once 6.7.  With a part for every piece of a group's channels
-// instead of one for all of them large groups are many parts: 30000 x 1023, three groups, forward 2690 us, now 106.)
+// instead of one for all of them large groups are many parts: 30000 x 1023, three groups, forward 2690 us, now 102.)
 constexpr int kHeldParts = 8;
 template <typename A, int LANES>
 __global__ __launch_bounds__(kNormBlock) void norm_stats_kernel(const A *__restrict__ parts, const int64_t *__restrict__ level_start, A *__restrict__ stats, NormDims d,

@@ -144,7 +144,8 @@ class SpatialCrossAttention_DFA3D(nn.Module):
         """``queries`` (bs, cams, L, E) plus the mean over the heads of the cells' rows of ``table`` (cells, heads, E), each scaled by what the sampling left unexplained
         (1 - ``update_weight`` (bs, cams, L, heads, 1)).  The rows that the lists name are read, scaled and added in one kernel; as tensor operations
         they are copied, masked, scaled, averaged and added, and their gradient is scattered: the layer of the base model with them, training 7252 -> 3482 us (without them
-        3197), inference 1523 -> 1088 (998).  More queries than cells are left to torch, whose indexing says so where one of them is seen."""
+        3197), inference 1523 -> 1088 (998).  That is float32 and float64 outside autocast: layers in bfloat16 or under autocast still take the
+        tensor operations.  More queries than cells are left to torch, whose indexing says so where one of them is seen."""
         bs, cams, L, _ = queries.shape
         if (num_query <= table.shape[0] and queries.dtype in (torch.float32, torch.float64) and ordinary(queries, update_weight, table, dtype=queries.dtype)
                 and update_weight.shape == (bs, cams, L, self.num_head, 1)):
