@@ -448,6 +448,7 @@ static bool ordered_at_once(int N, int V) { return V <= kOrderGroups * kOrderPer
 // at most two such entries, at its begin and at its end.
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 template <int HB> constexpr int kRunOf = HB == 1 ? 8 : 4;      // entries that a wavefront takes at the most
+constexpr int places_at_once(int hb) { return hb == 1 ? 4 : 1; }
 
 struct TableGrad {
   const void *table, *index, *scale, *grad;
@@ -491,7 +492,7 @@ template <typename T, int VEC, int HB, bool SCALED>
 __device__ __forceinline__ void add_places(const TableGrad &a, int from, int to, int first, int h0, int slice, int at, const typename Sum<T>::type (&t)[HB][VEC],
                                            typename Sum<T>::type (&sum)[HB][VEC]) {
   typedef typename Sum<T>::type A;
-  constexpr int kAtOnce = HB == 1 ? 4 : 1;                   // (with and without SCALED: it is the order of the sum)
+  constexpr int kAtOnce = places_at_once(HB);                // (with and without SCALED: it is the order of the sum)
   const A *scale = (const A *)a.scale;
   const int e = (slice * a.lanes + at) * VEC;
   const bool on = e < a.E, all_heads = h0 + HB <= a.H;
@@ -709,17 +710,24 @@ static int table_chunk(int N, int H, int E, int vec) {
 // at work while wavefronts add up one after the other many batch elements of each of an entry's places.  (Batch elements x places of entries x heads x elements in
 // float, gradients on the device: 1000 x 5 of 100 x 256 188 us of a pass and 47, 500 x 100 of 50 x 8 x 32 1912 and 62, 256 x 256 of 256 x 768 100 and 66, 64 x 250 of
 // 1000 x 256 31 and 26; 64 x 1000 of 1000 x 256 36 and 48, 32 x 300 of 300 x 8 x 256 37 and 44, 16 x 1000 of 1000 x 256 15 and 24.)
-// With more than 2^20 places in all, ordering them costs: there the pieces of an index of many places count as entries do.  (Likewise, gradients on the device, one
-// after the other and as places of their own: 20000 x 100 of 100 x 256 10191 us and 433, 2000 x 1000 of 1000 x 64 1075 and 212, 128 x 10000 of 100 x 256 481 and 292,
-// 16 x 100000 of 100 x 8 104 and 94; left one after the other 64 x 20000 of 100 x 256 290.)  And more than 2^20 batch elements always, as one float adds up those of
-// a place that are not places of their own.
+// With more than 2^20 places in all, ordering them costs as well: there both sides' times are weighed.  A wavefront's step takes some 1.2 us (bfloat16 by eights 2.5); one after
+// the other it makes them for all batch elements of an entry's or a piece's places; as places of their own a million takes 80 us to order, then g for all heads at the
+// rate of a copy or a piece's steps, and the join 1 us for 64 pieces of an entry.  (Likewise: 20000 x 100 of 100 x 256 10191 and 433, 1020 x 16747 of 266 x 8 x 68 15878 and
+// 3265, 300 x 4000 of 300 x 16 1512 and 104, 147 x 52107 of 323 x 4 817 and 475, 9 x 131072 of 900 x 2 x 4 145 and 125; 64 x 20000 of 100 x 256 290 and 340, 8 x 200000 of
+// 1000 x 4 107 and 143, 12 x 100000 of 100 x 8 x 64 244 and 362, 239 x 15296 of one of 16 634 and 1031.)  And more than 2^20 batch elements always, as one float adds
+// up those of a place that are not places of their own.
 constexpr long long kMostPlaces = 1LL << 30, kSerialElements = 1LL << 20;
 static bool spread_over(long long R, int N, int V, int H, int E, int vec) {
   if (R < 8 || R > kMostPlaces / N) return false;
-  const int lanes = table_lanes(E, vec), slices = (E + lanes * vec - 1) / (lanes * vec), hb = heads_at_once(H), entries = std::min(N, V);
-  const int runs = R * N > (1 << 20) ? std::max(entries, N / table_chunk(N, H, E, vec)) : entries;
-  const long long waves = (long long)runs * slices * ((H + hb - 1) / hb) / (kWave / lanes);
-  return R > kSerialElements || (R * N / entries >= 128 && waves < 1024);
+  if (R > kSerialElements) return true;
+  const int lanes = table_lanes(E, vec), slices = (E + lanes * vec - 1) / (lanes * vec), hb = heads_at_once(H), head_blocks = (H + hb - 1) / hb, entries = std::min(N, V);
+  if (R * N <= (1 << 20)) return R * N / entries >= 128 && (long long)entries * slices * head_blocks / (kWave / lanes) < 1024;
+  const double all = (double)R * N, step = vec == 8 ? 2.5 : 1.2;
+  auto steps = [&](int places) { return (places + places_at_once(hb) - 1) / places_at_once(hb); };
+  const int chunk = table_chunk((int)(R * N), H, E, vec);
+  const double serial = step * R * steps(std::min((N + entries - 1) / entries, table_chunk(N, H, E, vec)));
+  const double own = 25 + 80e-6 * all + std::max(all * head_blocks * E * 4 / 5.1e6, step * steps(chunk)) + all / chunk / entries / 64;
+  return serial > own;
 }
 // Batch elements that would have to be places of their own, and are more than can be.
 bool embedding_too_many(long long R, int N) { return R > kSerialElements && R > kMostPlaces / N; }
@@ -767,7 +775,7 @@ size_t embedding_workspace_bytes(long long R, int one, int V, int H, int E, int 
   // (whatever the operands' alignment turns out to be)
   const size_t elem = dtype == DFA3D_F64 ? 8 : 4;
   size_t most = 0;
-  for (int vec = 1; vec <= 8; vec *= 2) {
+  for (int vec = 1; vec <= (dtype == DFA3D_BF16 ? 8 : dtype == DFA3D_F32 ? 4 : 2); vec *= 2) {
     const int N = spread_over(R, one, V, H, E, vec) ? (int)(R * one) : one, chunk = table_chunk(N, H, E, vec);
     most = std::max(most, order_plan(N, V, nullptr).bytes + (N > chunk ? (size_t)((N + chunk - 1) / chunk) * 2 * H * E * elem : 0));
   }

@@ -21,7 +21,7 @@ def test_batch_elements_are_places_of_their_own():
     need = _lib.lib().dfa3d_embedding_grad_table_workspace_bytes
     for R, N, V, H, E in ((10000, 100, 100, 1, 256), (20000, 100, 100, 1, 256), (2 ** 25, 1, 1, 1, 8), (2 ** 21, 1, 9, 512, 512), (2 ** 30, 1, 1, 1, 1)):
         assert need(R, N, V, H, E, 0) == need(1, R * N, V, H, E, 0)
-    for R, N, V, H, E in ((7, 200000, 1, 1, 256), (64, 2 ** 20, 100, 1, 256), (64, 2000, 2000, 8, 256)):
+    for R, N, V, H, E in ((7, 200000, 1, 1, 256), (16, 2 ** 20, 2 ** 19, 1, 256), (64, 2000, 2000, 8, 256)):
         assert need(R, N, V, H, E, 0) == need(1, N, V, H, E, 0)
 
 
